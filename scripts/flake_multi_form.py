@@ -1,8 +1,7 @@
 """Round 5's one unexplained failure, reproduced in round 6 (scripts/flake_k16_suite_context.py, profiles/r06_flake2_context_3000.log:
 1 of 24 000 method-3 calls, in the DEVICE-LIST form with one device listed twice, 8 aligned pairs of one candidate at other positions):
 that form only, with the device listed FLAKE_DEVICES times (default 4: as many contexts working side by side on the one GPU), against
-results of the oracle computed once.  FLAKE_LIBRARY=<path of a libshasta_mi355x.so>: another build (the A/B with vector stores of the
-trace: make -C shasta_amd/csrc OUT=../_build_vector_stores EXTRA=-DSHASTA_TRACE_VECTOR_STORES=1).
+results of the oracle computed once.  FLAKE_LIBRARY=<path of a libshasta_mi355x.so>: another build.
     python scripts/flake_multi_form.py <repeats>"""
 import os
 import sys

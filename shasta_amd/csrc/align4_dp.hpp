@@ -327,11 +327,12 @@ template<int TIE> struct DpTie {
 //    to every cell is gone (9 -> 8 VALU instructions per cell);
 //  * trace planes: one ballot per comparison (the mask v_cmp wrote anyway), combined on the
 //    scalar unit; the ballot of a combined predicate is compiled to v_cndmask + v_cmp;
-//  * the trace record goes from the scalar registers the ballots are in straight to memory: scalar stores
-//    (s_store_dwordx4, RW / 2 per iteration), no vector instruction at all.  (Round 1 staged the 256-byte line in LDS:
-//    12 % of the wave cycles were LDS issue stalls; the first version of round 2 assembled it in one vector register
-//    with v_writelane_b32, 2 RW VALU instructions per iteration of a kernel bound by VALU issue: 8 of 31 for C = 2.
-//    scripts/microbench/trace_store.hip measured both ways of writing the same records: identical bytes, 0.84 -> 0.62 ms.)
+//  * the trace record goes from the scalar registers the ballots are in into the lanes of a vector register (v_writelane_b32: two
+//    per word, 8 of the 26 VALU instructions of an iteration for C = 2), and a 256-byte line leaves as one coalesced store
+//    (UniformWords).  The kernel is bound by VALU issue.  Against 16-byte stores of lane 0, RW / 2 per iteration (the same
+//    number of moves, but a change of EXEC and a branch around them in every iteration): 20 000 tasks of 1 500 markers
+//    6.2 -> 5.4 ms, the <= 64-diagonal class 540 -> 950 GCUPS.  Staging the line in LDS cost 12 % of the wave cycles in LDS
+//    issue stalls.
 //  * trip counts are made scalar (readfirstlane), so loop control runs on the scalar unit.
 constexpr int DP_BLOCK = 4;
 __device__ __forceinline__ uint64_t ballot64(bool p) { return __builtin_amdgcn_ballot_w64(p); }
@@ -398,7 +399,7 @@ bandedDpForwardKernel(
 #pragma unroll
     for(int d = 1; d < WAVE; d <<= 1) itersLane = max(itersLane, uint32_t(__shfl_xor(int(itersLane), d, WAVE)));
     const uint32_t iters = __builtin_amdgcn_readfirstlane(itersLane);
-    uint64_t* __restrict__ tr = uniformPointer(trace + bundleOffsets[bundle]);
+    uint64_t* __restrict__ tr = trace + uniformOffset(bundleOffsets[bundle]);
 
     // Per diagonal: first and last anti-diagonal that hold a cell of the matrix.
     int32_t lo[C];
@@ -471,16 +472,13 @@ bandedDpForwardKernel(
         }
     };
     // The record of iteration `it`: RW ballot words, uniform across the wavefront, in scalar registers; they go to
-    // tr[it RW ...] as they are.
+    // tr[it RW ...] as they are.  (The steady phase collects the records of a group.)
     auto putRecord = [&](uint32_t it, const uint64_t (&words)[RW]) {
         SHASTA_DEVICE_CHECK((uint64_t(it) + 1) * RW <= ((uint64_t(iters) * RW + 31) & ~31ULL));       // inside the bundle's trace (dpBundleKernel)
+        UniformWords<RW> record;
 #pragma unroll
-        for(int k = 0; k < RW; k += 2) scalarStore128(tr + uint64_t(it) * RW + k, words[k], words[k + 1]);
-    };
-    // The same for iteration `index` (a constant once the steady phase is unrolled) of the group whose records start at `base`.
-    auto putRecordOfGroup = [&](uint64_t* base, int index, const uint64_t (&words)[RW]) {
-#pragma unroll
-        for(int k = 0; k < RW; k += 2) scalarStore128At(base, (index * RW + k) * 8, words[k], words[k + 1]);
+        for(int k = 0; k < RW; k++) record.put(k, words[k]);
+        record.store(tr + uint64_t(it) * RW);
     };
 
     // General iterations [from, to): sliding register windows fed by clamped loads two iterations ahead.
@@ -557,6 +555,7 @@ bandedDpForwardKernel(
             uint64_t* groupRecords = tr + uint64_t(steadyBegin) * RW;
             SHASTA_DEVICE_CHECK((uint64_t(steadyBegin) + uint64_t(groups) * AL) * RW <= ((uint64_t(iters) * RW + 31) & ~31ULL));
             for(uint32_t grp = 0; grp < groups; grp++, groupRecords += AL * RW) {
+                UniformWords<AL * RW> records;
 #pragma unroll
                 for(int blk = 0; blk < AL / U; blk++) {
                     const int cur = blk & 1, nxt = cur ^ 1;
@@ -570,19 +569,20 @@ bandedDpForwardKernel(
                     for(int u = 0; u < U; u++) {
                         uint64_t words[RW];
                         antiDiagonals(phaseTag, geo.s0 + 2 * int32_t(steadyBegin + grp * AL + blk * U + u), [&](int k) { return a(u + k); }, [&](int h) { return e(u + HC - 1 - h); }, words);
-                        putRecordOfGroup(groupRecords, blk * U + u, words);
+#pragma unroll
+                        for(int k = 0; k < RW; k++) records.put((blk * U + u) * RW + k, words[k]);
                     }
 #pragma unroll
                     for(int x = 0; x < HC; x++) tailA[x] = a(x + U);
 #pragma unroll
                     for(int x = 0; x < HC - 1; x++) tailB[x] = e(x + U);
                 }
+                records.store(groupRecords);
             }
         };
         steady(DpPhase<true>{});
         general(steadyBegin + groups * AL, iters);
     }
-    scalarStoreFlush();                                   // the scalar data cache is write-back
 
     // End cell: maximum over the border cells = final value of every diagonal; ties by the policy (the reading: the smallest (i, j)).
     int32_t bestScore = NEG_SCORE, bestI = DpTie<TIE>::noEndCell, bestJ = DpTie<TIE>::noEndCell;

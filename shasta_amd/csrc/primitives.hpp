@@ -26,52 +26,47 @@ __device__ __forceinline__ uint32_t reverseComplementKmerId(uint32_t kmerId, uin
     return ((__brev(high) >> (32u - k)) << k) | (__brev(low) >> (32u - k));
 }
 
-// s_store_dwordx4: 16 bytes that live in scalar registers (wave-uniform by construction: ballots) go to global memory without
-// passing through a vector register.  `address` must be wave-uniform (an SGPR pair) and 4-byte aligned.  The scalar data cache
-// is write-back: scalarStoreFlush() before the wavefront ends, or a later kernel may not see the data.
-// (The wave64 emulator of tests/emu supplies its own: SHASTA_SCALAR_STORE_DEFINED.)
-#if !defined(SHASTA_SCALAR_STORE_DEFINED) && defined(SHASTA_TRACE_VECTOR_STORES)
-// (the same three entry points as plain vector stores of lane 0: the A/B build of the search for round 5's method-3 failure, and the
-// form to fall back on should scalar stores ever be at fault -- make OUT=../_build_vector_stores EXTRA=-DSHASTA_TRACE_VECTOR_STORES=1)
-#define SHASTA_SCALAR_STORE_DEFINED
-__device__ __forceinline__ void scalarStore128(void* address, uint64_t low, uint64_t high)
-{
-    if(laneId() == 0) *reinterpret_cast<uint4*>(address) = make_uint4(uint32_t(low), uint32_t(low >> 32), uint32_t(high), uint32_t(high >> 32));
-}
-__device__ __forceinline__ void scalarStore128At(void* address, int byteOffset, uint64_t low, uint64_t high)
-{
-    scalarStore128(static_cast<char*>(address) + byteOffset, low, high);
-}
-__device__ __forceinline__ void scalarStoreFlush() {}
-template<class T> __device__ __forceinline__ T* uniformPointer(T* p)
-{
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
-    return reinterpret_cast<T*>((uint64_t(hi) << 32) | lo);
-}
+// v_writelane_b32: `v` (uniform) into the lane `lane` (uniform) of `old`.  The compiler's own intrinsic, which clang has no builtin for:
+// unlike inline assembly it is scheduled with the waits that a scalar register written by a comparison needs before it is read.
+// (The wave64 emulator of tests/emu has its own.)
+#ifdef __HIPCC__
+extern "C" __device__ uint32_t writeLane(uint32_t v, uint32_t lane, uint32_t old) __asm("llvm.amdgcn.writelane.i32");
 #endif
-#ifndef SHASTA_SCALAR_STORE_DEFINED
-__device__ __forceinline__ void scalarStore128(void* address, uint64_t low, uint64_t high)
+// WORDS 64-bit words that are the same in every lane (ballots: they live in scalar registers) on their way to consecutive global
+// memory: word k goes into lanes 2 k and 2 k + 1 of a line of 32 words (v_writelane_b32, two per word), a line leaves as one
+// coalesced vector store of four bytes per lane.  `k` is a constant once the caller's loops are unrolled; every lane of the
+// wavefront takes part in every call.
+template<int WORDS> struct UniformWords {
+    static constexpr int LINES = (WORDS + 31) / 32;
+    uint32_t line[LINES];
+    __device__ __forceinline__ UniformWords()
+    {
+#pragma unroll
+        for(int n = 0; n < LINES; n++) line[n] = 0;
+    }
+    __device__ __forceinline__ void put(int k, uint64_t word)
+    {
+        uint32_t& r = line[k / 32];
+        r = writeLane(uint32_t(word), 2 * (k % 32), r);
+        r = writeLane(uint32_t(word >> 32), 2 * (k % 32) + 1, r);
+    }
+    __device__ __forceinline__ void store(uint64_t* address) const
+    {
+        uint32_t* const out = reinterpret_cast<uint32_t*>(address) + laneId();
+#pragma unroll
+        for(int n = 0; n < LINES; n++) {
+            const int dwords = 2 * WORDS - 64 * n;             // (the last line may be a short one)
+            if(dwords >= 64 || laneId() < dwords) out[64 * n] = line[n];
+        }
+    }
+};
+// A wave-uniform offset the compiler cannot prove uniform (it depends on threadIdx.x >> 6), in scalar registers.  (Of the offset, not of
+// the pointer: a pointer rebuilt from integers has lost its address space, and a flat store makes every later load wait for it.)
+__device__ __forceinline__ uint64_t uniformOffset(uint64_t v)
 {
-    const __uint128_t v = (__uint128_t(high) << 64) | __uint128_t(low);
-    asm volatile("s_store_dwordx4 %0, %1, 0x0" :: "s"(v), "s"(address) : "memory");
-}
-// The same at a byte offset that is a constant by the time the code is generated (an expression of unrolled loop counters):
-// it goes into the instruction, no address arithmetic.
-__device__ __forceinline__ void scalarStore128At(void* address, int byteOffset, uint64_t low, uint64_t high)
-{
-    const __uint128_t v = (__uint128_t(high) << 64) | __uint128_t(low);
-    asm volatile("s_store_dwordx4 %0, %1, %2" :: "s"(v), "s"(address), "i"(byteOffset) : "memory");
-}
-__device__ __forceinline__ void scalarStoreFlush() { asm volatile("s_dcache_wb\n\ts_waitcnt lgkmcnt(0)" ::: "memory"); }
-// A wave-uniform pointer the compiler cannot prove uniform (it depends on threadIdx.x >> 6).
-template<class T> __device__ __forceinline__ T* uniformPointer(T* p)
-{
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
     const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
-    return reinterpret_cast<T*>((uint64_t(hi) << 32) | lo);
+    return (uint64_t(hi) << 32) | lo;
 }
-#endif
 
 // An element count a kernel is given: an upper bound known on the host (grids are sized from it) and, optionally, the
 // address of the exact count on the device, written by an earlier kernel of the same stream.  The host never reads the

@@ -232,6 +232,12 @@ __forceinline__ uint32_t __builtin_amdgcn_readfirstlane(uint32_t v)
     return uint32_t(hipemu::collective(hipemu::FIRSTLANE, v, 0));
 }
 
+// v_writelane_b32 (primitives.hpp declares the device's): `v` (uniform) into the lane `lane` (uniform) of `old`.
+__forceinline__ uint32_t writeLane(uint32_t v, uint32_t lane, uint32_t old)
+{
+    return (uint32_t(threadIdx.x) & 63u) == (lane & 63u) ? v : old;
+}
+
 __forceinline__ int __popc(unsigned v) { return __builtin_popcount(v); }
 __forceinline__ int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 __forceinline__ int __ffs(int v) { return __builtin_ffs(v); }
@@ -252,15 +258,6 @@ __forceinline__ uint32_t __builtin_amdgcn_alignbyte(uint32_t hi, uint32_t lo, ui
 {
     return uint32_t(((uint64_t(hi) << 32) | uint64_t(lo)) >> (8u * (c & 3u)));
 }
-// s_store_dwordx4 + s_dcache_wb (inline assembly in primitives.hpp): lane 0 of the wavefront stores.
-#define SHASTA_SCALAR_STORE_DEFINED 1
-__forceinline__ void scalarStore128(void* address, uint64_t low, uint64_t high)
-{
-    if((uint32_t(threadIdx.x) & 63u) == 0) { uint64_t v[2] = {low, high}; std::memcpy(address, v, 16); }
-}
-__forceinline__ void scalarStore128At(void* address, int byteOffset, uint64_t low, uint64_t high) { scalarStore128(static_cast<char*>(address) + byteOffset, low, high); }
-__forceinline__ void scalarStoreFlush() {}
-template<class T> __forceinline__ T* uniformPointer(T* p) { return p; }
 #ifndef __clang__
 template<class T> __forceinline__ T __hip_atomic_load(const T* p, int, int) { return __atomic_load_n(p, __ATOMIC_RELAXED); }
 #endif
