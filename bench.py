@@ -946,8 +946,14 @@ def main():
     ctx.close()
     if final_line is not None and retry_with:
         sys.stderr.write("bench.py: the parity check at bench size FAILED on this path; running again with %s\n" % {k: v for k, v in retry_with.items() if k in FALLBACK_SWITCHES})
-        _flush_all_stdio()
-        os.execve(sys.executable, [sys.executable] + sys.argv, dict(os.environ, **retry_with))
+        code = _run_again(retry_with)
+        if code == 0:
+            return
+        # The fallback did not get to a line of its own: the failed path's line is what there is (its mismatches are in it), and the
+        # exit code says that it is no measurement.
+        out["fallback_exit_code"] = code
+        print(json.dumps(headline(out, write_details(out)), allow_nan=False), flush=True)
+        sys.exit(code)
     if dist is not None:
         # The JSON line has to be the LAST thing on stdout: RCCL's version banner (it prints one when NCCL_DEBUG asks for it, as
         # on the GPU box) sits in the C library's stdout buffer of a process until that is flushed -- at exit, i.e. AFTER a line
@@ -1039,7 +1045,7 @@ def headline(out, details_path):
     if u:
         # What a one-shot call of the seams pays in addition (the markers cross PCIe on every call): never `value`.
         line["pcie_inclusive"] = {k: u.get(k) for k in ("value_with_upload_every_step", "upload_seconds")}
-    for k in ("parity_at_bench_size", "speedup_vs_cpu_baseline", "stage_seconds_per_step", "aligner_status", "path", "default_path_parity_failed"):
+    for k in ("parity_at_bench_size", "speedup_vs_cpu_baseline", "stage_seconds_per_step", "aligner_status", "path", "default_path_parity_failed", "fallback_exit_code"):
         if out.get(k) is not None:
             line[k] = out[k]
     h = out.get("hbm_natured_kernel")
@@ -1120,8 +1126,7 @@ def _flush_all_stdio():
 
 
 # The library's own switches back to earlier forms of its kernels: what the line falls back on, one step at a time,
-# when the parity check at bench size fails or the library raises -- round 4's kernels had not run on a GPU when they were
-# committed.  The line then says so (`path`, `earlier_attempts`): it is the same work on the same reads through kernels that
+# when the parity check at bench size or one of the library's own checks fails.  The line then says so (`path`, `earlier_attempts`): it is the same work on the same reads through kernels that
 # produce the same results, never a skipped stage, and never silent.
 FALLBACK_SWITCHES = ("SHASTA_MI355X_ANCHORED_DP", "SHASTA_MI355X_SPARSE_DP", "SHASTA_MI355X_STATISTICS_ATOMICS")
 
@@ -1145,20 +1150,42 @@ def _fallback_environment(parity, error):
     return switches or None
 
 
+def _library_check_failed(error):
+    """One of the library's own consistency checks (MI355X_ASSERT): every call of the runtime up to it had succeeded.  Whatever else it
+    raises -- an error of the HIP runtime or of RCCL above all -- may have left the device at fault, and nothing more is started on it."""
+    return "Assertion failed: " in str(error) and "HIP error" not in str(error)
+
+
+def _run_again(retry_with):
+    """This script again, in a process of its own with `retry_with` in its environment; its line becomes this process's.  -> 0, or the
+    exit code to end with (no line was printed).  A process that has initialised the GPU must not be replaced by another program."""
+    import subprocess
+    _flush_all_stdio()
+    child = subprocess.run([sys.executable] + sys.argv, env=dict(os.environ, **retry_with), stdout=subprocess.PIPE, text=True)
+    if child.returncode == 0 and any(line.startswith("{") for line in child.stdout.splitlines()):
+        print(child.stdout, end="", flush=True)
+        return 0
+    sys.stderr.write("bench.py: the run with %s ended with code %d: %s\n" % ({k: v for k, v in retry_with.items() if k in FALLBACK_SWITCHES}, child.returncode, child.stdout[-2000:]))
+    return child.returncode if child.returncode > 0 else 1
+
+
 def _main_with_safety_net():
     try:
         main()
-    except (RuntimeError, AssertionError) as e:
+        return
+    except RuntimeError as e:
         single = int(os.environ.get("WORLD_SIZE", "1")) == 1 and "--group" not in sys.argv
-        retry_with = _fallback_environment(None, e) if single else None
+        retry_with = _fallback_environment(None, e) if single and _library_check_failed(e) else None
         if not retry_with:
             raise
         attempts = json.loads(os.environ.get("SHASTA_BENCH_EARLIER_ATTEMPTS", "[]"))
         attempts.append({"switches": {k: os.environ[k] for k in FALLBACK_SWITCHES if k in os.environ}, "raised": str(e)[:400]})
         retry_with["SHASTA_BENCH_EARLIER_ATTEMPTS"] = json.dumps(attempts)
         sys.stderr.write("bench.py: the library raised (%s); running again with %s\n" % (str(e)[:200], {k: v for k, v in retry_with.items() if k in FALLBACK_SWITCHES}))
-        _flush_all_stdio()
-        os.execve(sys.executable, [sys.executable] + sys.argv, dict(os.environ, **retry_with))
+    # (Outside the handler: the failed run's frames, and with them its context's device memory, are gone.)
+    code = _run_again(retry_with)
+    if code:
+        sys.exit(code)
 
 
 if __name__ == "__main__":

@@ -319,3 +319,86 @@ def test_fallback_switches_one_step_at_a_time(monkeypatch):
     assert bench._fallback_environment(dict(good, aligner_mismatches=1), None) is None               # nothing left to switch: the line stands as it is
     monkeypatch.delenv("SHASTA_MI355X_ANCHORED_DP"); monkeypatch.delenv("SHASTA_MI355X_SPARSE_DP")
     assert bench._fallback_environment(None, RuntimeError("HIP error")) == {"SHASTA_MI355X_STATISTICS_ATOMICS": "1", "SHASTA_MI355X_SPARSE_DP": "0"}
+
+
+# ---- the safety net's second run is a process of its own ------------------------------------------------------------------
+
+EXEC_REFUSED = ("import os, runpy, sys\n"
+                "def refused(*args):\n    raise SystemExit('this process was about to be replaced')\n"
+                "os.execv = os.execve = os.execvp = os.execvpe = refused\n"
+                "sys.argv = sys.argv[1:]\n"
+                "runpy.run_path(sys.argv[0], run_name='__main__')\n")
+
+
+def test_the_fallback_runs_where_a_process_may_not_be_replaced(emu_lib):
+    import os
+    import subprocess
+    import tempfile
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    details = os.path.join(tempfile.mkdtemp(), "details.json")
+    env = dict(os.environ, SHASTA_BENCH_LIBRARY=emu_lib.path, SHASTA_BENCH_FORCE_PARITY_FAILURE="1", SHASTA_BENCH_DETAILS=details)
+    out = subprocess.run([sys.executable, "-c", EXEC_REFUSED, os.path.join(root, "bench.py"), "--reads", "100", "--steps", "1", "--warmup", "0", "--no-cpu-baseline"],
+                         env=env, capture_output=True, text=True, timeout=1500)
+    assert out.returncode == 0, out.stderr[-2000:]
+    lines = [line for line in out.stdout.splitlines() if line.startswith("{")]
+    assert len(lines) == 1
+    head = strict_loads(lines[0])
+    assert "SHASTA_MI355X_ANCHORED_DP=0" in head["path"] and len(head["earlier_attempts"]) == 1 and "fallback_exit_code" not in head
+
+
+def test_a_failing_fallback_leaves_the_failed_line_and_its_exit_code(emu_lib):
+    """The second run cannot work (its library does not exist): the first one's line is printed, alone, with the code it ends with."""
+    import os
+    import subprocess
+    import tempfile
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    details = os.path.join(tempfile.mkdtemp(), "details.json")
+    prepare = "import subprocess as s\nrun = s.run\ns.run = lambda a, **k: run(a, **dict(k, env=dict(k['env'], SHASTA_BENCH_LIBRARY='/nonexistent.so')) if 'env' in k else k)\n"
+    env = dict(os.environ, SHASTA_BENCH_LIBRARY=emu_lib.path, SHASTA_BENCH_FORCE_PARITY_FAILURE="1", SHASTA_BENCH_DETAILS=details)
+    out = subprocess.run([sys.executable, "-c", prepare + EXEC_REFUSED, os.path.join(root, "bench.py"), "--reads", "100", "--steps", "1", "--warmup", "0", "--no-cpu-baseline"],
+                         env=env, capture_output=True, text=True, timeout=1500)
+    lines = [line for line in out.stdout.splitlines() if line.startswith("{")]
+    assert out.returncode != 0 and len(lines) == 1, out.stderr[-2000:]
+    head = strict_loads(lines[0])
+    assert head["fallback_exit_code"] == out.returncode and head["value"] > 0 and "path" not in head
+    assert strict_loads(open(details).read())["fallback_exit_code"] == out.returncode
+
+
+@pytest.mark.parametrize("message, runs_again", [
+    ("align4_run_borrowed failed: Assertion failed: rows == stored at align4.hip:1", True),
+    ("align4_run_borrowed failed: HIP error: unspecified launch failure in hipStreamSynchronize(stream) at align4.hip:1", False),
+    ("lowhash0_run failed: HIP error: out of memory in hipMalloc(&q, bytes) at common.hpp:1", False),
+    ("group: RCCL error in ncclSend: unhandled cuda error", False),
+    ("Align4: invalid alignment candidate (need readId0 < readId1 < readCount).", False),
+])
+def test_nothing_more_is_started_after_an_error_of_the_device(monkeypatch, message, runs_again):
+    import os
+    import subprocess
+    import types
+    import bench
+    for k in bench.FALLBACK_SWITCHES + ("SHASTA_BENCH_FORCE_PARITY_FAILURE", "SHASTA_BENCH_EARLIER_ATTEMPTS", "WORLD_SIZE"):
+        monkeypatch.delenv(k, raising=False)
+    started = []
+
+    def fail():
+        raise RuntimeError(message)
+
+    def run(command, **keywords):
+        started.append(keywords["env"])
+        return types.SimpleNamespace(returncode=0, stdout="{}\n")
+
+    def replaced(*args):
+        raise SystemExit("this process was about to be replaced")
+
+    monkeypatch.setattr(bench, "main", fail)
+    monkeypatch.setattr(subprocess, "run", run)
+    monkeypatch.setattr(os, "execve", replaced)
+    monkeypatch.setattr(sys, "argv", ["bench.py"])
+    if runs_again:
+        bench._main_with_safety_net()
+        assert len(started) == 1 and started[0]["SHASTA_MI355X_SPARSE_DP"] == "0"
+        assert json.loads(started[0]["SHASTA_BENCH_EARLIER_ATTEMPTS"])[0]["raised"] == message
+    else:
+        with pytest.raises(RuntimeError, match="error|invalid"):
+            bench._main_with_safety_net()
+        assert started == []
