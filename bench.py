@@ -257,7 +257,7 @@ def cpu_baseline(ctx, toc, kmer, p, o, align_method, gpu_lowhash, sample_size, c
         t_suppress = time.time() - t0
     # Assembler::computeSortedMarkers (src/AssemblerAlign.cpp:236-239): once, for all oriented reads, before the alignment threads
     # start -- timed on its own; the per-candidate loop below reads it (method 4; method 3 does not use sorted markers).
-    t_sorted = lib.compute_sorted_markers(toc, data7, threads=cores) if (kind == "reference" and align_method == 4) else 0.0
+    t_sorted = lib.compute_sorted_markers(toc, data7, threads=cores) if align_method == 4 else 0.0
     parity["lowhash0_candidates"] = len(lh.candidates)
     if suppress is not None:
         parity["candidates_after_suppression"] = len(cand)
@@ -280,19 +280,15 @@ def cpu_baseline(ctx, toc, kmer, p, o, align_method, gpu_lowhash, sample_size, c
     per_pair = (t2 - t1) / (len(sample) - len(small)) if (not whole and len(sample) > len(small)) else 0.0
     if per_pair <= 0.0:                                 # the whole list, or too few candidates for the difference to mean anything
         per_pair = t2 / max(1, len(sample))
-    if kind == "reference":
-        lib.drop_sorted_markers()
+    lib.drop_sorted_markers()
     dev = (ctx.align4 if align_method == 4 else ctx.align3)(sample, o, want_ordinals=True, borrow=True)
     # Assembler::computeAlignmentTable (src/AssemblerAlign.cpp:296, 509-571; serial in the reference) on the alignments of the
     # WHOLE candidate list -- the device's rows of the bench's last step (equal to the reference's wherever both exist, below) --
     # and compared with the table the device made from the sample's.
-    t_table = 0.0
-    if kind == "reference":
-        sample_toc, sample_values = ctx.alignment_table()
-        ref_toc, ref_values, _ = lib.alignment_table(np.array(dev.alignment_data, copy=True), (len(toc) - 1) // 2)
-        parity["alignment_table_equal"] = bool(np.array_equal(sample_toc, ref_toc) and np.array_equal(sample_values, ref_values))
-        if all_rows is not None:
-            t_table = lib.alignment_table(all_rows, (len(toc) - 1) // 2)[2]
+    sample_toc, sample_values = ctx.alignment_table()
+    ref_toc, ref_values, _ = lib.alignment_table(np.array(dev.alignment_data, copy=True), (len(toc) - 1) // 2)
+    parity["alignment_table_equal"] = bool(np.array_equal(sample_toc, ref_toc) and np.array_equal(sample_values, ref_values))
+    t_table = lib.alignment_table(all_rows, (len(toc) - 1) // 2)[2] if all_rows is not None else 0.0
     ties = (ref.status & 0x80) != 0
     parity["aligner_sampled_candidates"] = len(sample)
     parity["aligner_ties_in_sample"] = int(ties.sum())

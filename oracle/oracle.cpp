@@ -107,6 +107,77 @@ void oracle_lowhash0_free(shasta_lowhash0_result* r)
     std::memset(r, 0, sizeof(*r));
 }
 
+// Assembler::computeSortedMarkers (src/AssemblerAlign4.cpp:190-261): all oriented reads once, before the alignment threads start.
+// oracle_align4_batch calls on the SAME markers then read it; without it they sort the two reads of every candidate.
+namespace {
+struct {
+    SortedMarkers sorted;
+    const void* markersData = nullptr;
+    uint64_t readCount = 0, markerCount = 0;
+} sortedMarkers;
+}
+
+int oracle_compute_sorted_markers(uint64_t readCount, const uint64_t* markersToc, const void* markersData, uint64_t threadCount, double* seconds)
+{
+    try {
+        const auto t0 = std::chrono::steady_clock::now();
+        const uint64_t markerCount = markersToc[2 * readCount];
+        std::vector<uint32_t> kmerIds;
+        extractKmerIds(static_cast<const uint8_t*>(markersData), markerCount, kmerIds);
+        sortedMarkers.markersData = nullptr;
+        sortedMarkers.sorted.resize(markerCount);
+        std::atomic<uint64_t> next(0);
+        auto work = [&]() {
+            for(;;) {
+                const uint64_t begin = next.fetch_add(1000);
+                if(begin >= 2 * readCount) break;
+                for(uint64_t i = begin; i < std::min(2 * readCount, begin + 1000); i++)
+                    sortMarkers(kmerIds.data() + markersToc[i], uint32_t(markersToc[i + 1] - markersToc[i]), sortedMarkers.sorted.data() + markersToc[i]);
+            }
+        };
+        std::vector<std::thread> threads;
+        for(uint64_t t = 1; t < (threadCount ? threadCount : std::thread::hardware_concurrency()); t++) threads.emplace_back(work);
+        work();
+        for(auto& t : threads) t.join();
+        sortedMarkers.markersData = markersData; sortedMarkers.readCount = readCount; sortedMarkers.markerCount = markerCount;
+        if(seconds) *seconds = std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
+        return 0;
+    } catch(std::exception& e) { lastError = e.what(); return 1; }
+}
+
+void oracle_drop_sorted_markers()
+{
+    sortedMarkers.markersData = nullptr;
+    SortedMarkers().swap(sortedMarkers.sorted);
+}
+
+// Assembler::computeAlignmentTable (src/AssemblerAlign.cpp:509-571): an alignment is listed under its two oriented reads and under
+// their reverse complements, every list ordered by (the other oriented read, alignment index).
+int oracle_alignment_table(uint64_t readCount, uint64_t alignmentCount, const shasta_alignment_data* rows, uint64_t* toc, uint32_t* values, double* seconds)
+{
+    try {
+        const auto t0 = std::chrono::steady_clock::now();
+        std::vector< std::vector< std::pair<uint32_t, uint32_t> > > lists(2 * readCount);
+        for(uint64_t i = 0; i < alignmentCount; i++) {
+            const shasta_oriented_read_pair& p = rows[i].pair;
+            const uint32_t a = 2 * p.readIds[0], b = 2 * p.readIds[1] + (p.isSameStrand ? 0 : 1);
+            for(uint32_t strand = 0; strand < 2; strand++) {
+                lists.at(a ^ strand).emplace_back(b ^ strand, uint32_t(i));
+                lists.at(b ^ strand).emplace_back(a ^ strand, uint32_t(i));
+            }
+        }
+        uint64_t n = 0;
+        toc[0] = 0;
+        for(uint64_t k = 0; k < 2 * readCount; k++) {
+            std::sort(lists[k].begin(), lists[k].end());
+            for(const auto& entry : lists[k]) values[n++] = entry.second;
+            toc[k + 1] = n;
+        }
+        if(seconds) *seconds = std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
+        return 0;
+    } catch(std::exception& e) { lastError = e.what(); return 1; }
+}
+
 int oracle_align4_batch(
     uint64_t readCount, const uint64_t* markersToc, const void* markersData,
     uint64_t candidateCount, const shasta_oriented_read_pair* candidates,
@@ -127,6 +198,8 @@ int oracle_align4_batch(
 
         struct PerCandidate { Ordinals ord; Info info; uint8_t status; uint64_t dpCells; };
         std::vector<PerCandidate> per(candidateCount);
+        const bool sorted = sortedMarkers.markersData == markersData && sortedMarkers.readCount == readCount && sortedMarkers.markerCount == markersToc[2 * readCount] && markersData;
+        auto sortedOf = [&](uint64_t orientedRead) { return sorted ? sortedMarkers.sorted.data() + markersToc[orientedRead] : nullptr; };
         const uint64_t threadCount = std::max<uint64_t>(1, threadCountSetting.load());
         std::atomic<uint64_t> next(0);
         auto work = [&]() {
@@ -143,7 +216,7 @@ int oracle_align4_batch(
                     const uint32_t ny = uint32_t(markersToc[or1 + 1] - markersToc[or1]);
                     PerCandidate& pc = per[i];
                     align4(kmerIds.data() + markersToc[or0], nx, kmerIds.data() + markersToc[or1], ny,
-                        opt, pc.ord, pc.info, &trace);
+                        opt, pc.ord, pc.info, &trace, sortedOf(or0), sortedOf(or1));
                     pc.dpCells = trace.dpCells;
                     if(pc.ord.empty()) pc.status = SHASTA_ALIGN_EMPTY;
                     else pc.status = passesOuterFilters(pc.ord, pc.info, opt, o->suppressContainments != 0) ?

@@ -443,32 +443,39 @@ inline void getxy(uint32_t X, uint32_t Y, uint32_t nx, int32_t& x, int32_t& y)
     y = (Xs + Ys - int32_t(nx) + 1) / 2;
 }
 
+// An oriented read's markers as (kmerId, ordinal), sorted by kmerId: src/AssemblerAlign4.cpp:243-258.
+using SortedMarkers = std::vector< std::pair<uint32_t, uint32_t> >;
+inline void sortMarkers(const uint32_t* k, uint32_t n, std::pair<uint32_t, uint32_t>* sorted)
+{
+    for(uint32_t i = 0; i < n; i++) sorted[i] = std::make_pair(k[i], i);
+    std::sort(sorted, sorted + n, [](const std::pair<uint32_t, uint32_t>& a, const std::pair<uint32_t, uint32_t>& b) { return a.first < b.first; });
+}
+
+// sorted0 / sorted1: sortMarkers of the two reads where the caller has it (once for all candidates, as the reference does).
 inline void align4(
     const uint32_t* k0, uint32_t nx, const uint32_t* k1, uint32_t ny,
-    const Align4Options& o, Ordinals& bestOrdinals, Info& bestInfo, Align4Trace* traceOut = nullptr)
+    const Align4Options& o, Ordinals& bestOrdinals, Info& bestInfo, Align4Trace* traceOut = nullptr,
+    const std::pair<uint32_t, uint32_t>* sorted0 = nullptr, const std::pair<uint32_t, uint32_t>* sorted1 = nullptr)
 {
     const uint32_t deltaX = uint32_t(int32_t(o.deltaX)), deltaY = uint32_t(int32_t(o.deltaY));
 
     // createAlignmentMatrix (:195-267): only the number of entries per cell matters downstream.
-    std::vector< std::pair<uint32_t, uint32_t> > s0(nx), s1(ny);       // (kmerId, ordinal), src/AssemblerAlign4.cpp:243-258
-    for(uint32_t i = 0; i < nx; i++) s0[i] = std::make_pair(k0[i], i);
-    for(uint32_t i = 0; i < ny; i++) s1[i] = std::make_pair(k1[i], i);
-    auto byKmer = [](const std::pair<uint32_t,uint32_t>& a, const std::pair<uint32_t,uint32_t>& b) { return a.first < b.first; };
-    std::sort(s0.begin(), s0.end(), byKmer);
-    std::sort(s1.begin(), s1.end(), byKmer);
+    SortedMarkers own0, own1;
+    if(!sorted0) { own0.resize(nx); sortMarkers(k0, nx, own0.data()); sorted0 = own0.data(); }
+    if(!sorted1) { own1.resize(ny); sortMarkers(k1, ny, own1.data()); sorted1 = own1.data(); }
     std::map< std::pair<uint32_t, uint32_t>, uint64_t > cellCount;     // key (iY, iX)
     {
         size_t i0 = 0, i1 = 0;
-        while(i0 < s0.size() && i1 < s1.size()) {
-            if(s0[i0].first < s1[i1].first) ++i0;
-            else if(s1[i1].first < s0[i0].first) ++i1;
+        while(i0 < nx && i1 < ny) {
+            if(sorted0[i0].first < sorted1[i1].first) ++i0;
+            else if(sorted1[i1].first < sorted0[i0].first) ++i1;
             else {
-                const uint32_t kmerId = s0[i0].first;
+                const uint32_t kmerId = sorted0[i0].first;
                 size_t e0 = i0, e1 = i1;
-                while(e0 < s0.size() && s0[e0].first == kmerId) ++e0;
-                while(e1 < s1.size() && s1[e1].first == kmerId) ++e1;
+                while(e0 < nx && sorted0[e0].first == kmerId) ++e0;
+                while(e1 < ny && sorted1[e1].first == kmerId) ++e1;
                 for(size_t a = i0; a < e0; a++) for(size_t b = i1; b < e1; b++) {
-                    const uint32_t x = s0[a].second, y = s1[b].second;
+                    const uint32_t x = sorted0[a].second, y = sorted1[b].second;
                     const uint32_t X = x + y, Y = nx + y - x - 1;                 // getXY :171-177
                     ++cellCount[std::make_pair(Y / deltaY, X / deltaX)];
                 }
