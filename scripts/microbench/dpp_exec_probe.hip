@@ -2,7 +2,7 @@
 // without a diagonal switched off instead of masking their values.  Lanes with (lane % 4 == 3) leave
 // before the DPP instruction; every other lane reads its neighbour below and above, with bound_ctrl on (zero fill) and off
 // (keep `old` = 0x55).  Prints one JSON line per variant with the 64 values.
-//     hipcc --offload-arch=gfx950 -O2 -o shasta_amd/_build/dpp_exec_probe scripts/microbench/dpp_exec_probe.hip
+//     hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o shasta_amd/_build/dpp_exec_probe scripts/microbench/dpp_exec_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

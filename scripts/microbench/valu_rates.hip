@@ -1,7 +1,7 @@
 // Issue rate of the integer instructions the window hash and the cells kernel lean on, measured on the device
 // (gfx950): independent chains per lane, enough waves to fill every SIMD; prints wave-instructions per cycle per CU
 // next to v_add_u32 (full rate = 4 SIMDs x 1 wave-instruction per 4 cycles... on the 16-lane SIMD of CDNA).
-// Build: hipcc --offload-arch=gfx950 -O3 -o shasta_amd/_build/valu_rates scripts/microbench/valu_rates.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o shasta_amd/_build/valu_rates scripts/microbench/valu_rates.hip
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

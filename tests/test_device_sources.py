@@ -4,6 +4,7 @@ assembly: every instruction in it is a VALU instruction or one of the few scalar
 import glob
 import os
 import re
+import subprocess
 
 import pytest
 
@@ -42,3 +43,10 @@ def test_inline_assembly_writes_no_memory(path):
     mnemonics = assembly_mnemonics(text)
     assert len(STATEMENT.findall(without_comments(text))) == len(re.findall(r"\b(?:asm|__asm__|__asm)\b", without_comments(text)))      # (none is left unread)
     assert [m for m in mnemonics if not (m.startswith("v_") or m in REGISTERS_ONLY)] == []
+
+
+def test_every_device_source_is_compiled_without_packed_fp32_instructions():
+    lines = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "shasta_amd", "csrc")], capture_output=True, text=True, check=True).stdout.splitlines()
+    compiled = [line for line in lines if "hipcc" in line and " -c " in line]
+    assert sorted(re.search(r"-c (\S+\.hip)", line).group(1) for line in compiled) == sorted(os.path.basename(path) for path in SOURCES if path.startswith("shasta_amd/csrc") and path.endswith(".hip"))
+    assert all("-Xclang -target-feature -Xclang -packed-fp32-ops" in line for line in compiled)
