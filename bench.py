@@ -44,10 +44,11 @@ HBM_PEAK_GBS = 8000.0          # /opt/skills/guides/MI355X_MICROARCH.md: 8.0 TB/
 # 1.35-1.55 of the 2 instructions per cycle and CU (scripts/microbench/valu_rates.hip, profiles/r02_valu_rates.jsonl).
 VALU_PEAK_WAVE_INSTRUCTIONS_PER_S = 256 * 4 * 0.5 * 2.4e9
 def _latest_pmc_file():
-    # The newest round's counter summary (profiles/rNN_pmc_100k_reads.json, written by scripts/gpu_profile.sh).
+    # The counter summary of the current build, or the newest of the numbered ones (scripts/pmc_summary.py writes both).
     import glob
+    current = os.path.join(ROOT, "profiles", "pmc_100k_reads.json")
     files = sorted(glob.glob(os.path.join(ROOT, "profiles", "r[0-9][0-9]_pmc_100k_reads.json")))
-    return files[-1] if files else os.path.join(ROOT, "profiles", "r02_pmc_100k_reads.json")
+    return current if os.path.exists(current) or not files else files[-1]
 
 
 PMC_FILE = _latest_pmc_file()
